@@ -1093,6 +1093,8 @@ struct Sampler {
       if (tid < ranks) of(&s, tid)->top[rank] = best;
       sync_all();
       for (int r = 0; r < ranks; ++r) best = max64(best, s.top[r]);
+    } else {
+      __syncthreads();  // every warp has read s.part: a search without a filter writes it next
     }
     top = from_ordered(uint32_t(best >> 32));
     inverse = kLog2e / t;

@@ -290,3 +290,25 @@ def test_top_p_in_large_batches(cuda):
     p = [1.0 if r % 3 == 0 else 0.5 + 0.49 * (r % 11) / 10 for r in range(rows)]
     m = [0.05 if r % 4 == 0 else 0.0 for r in range(rows)]
     _check(logits, t, k, p, m, _u(rows, 8))
+
+
+@pytest.mark.parametrize("vocab", [9, 40, 700, 8000])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_rows_of_one_cta_agree_on_their_largest_logit(cuda, vocab, infinite):
+    """Without a filter, and with an infinite logit, a row goes from its largest logit straight to the
+    sums, which use the same shared words; in a short row most warps have no logits and arrive early.
+    The other logits lie 60 below the largest (e^-60 has no weight), so the answer is known."""
+
+    from layer_streaming import ops
+
+    rows = 2000
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    best = torch.randint(0, vocab, (rows, 1), generator=gen, device="cuda")
+    logits = torch.rand((rows, vocab), generator=gen, device="cuda") - 62.0
+    logits.scatter_(1, best, float("inf") if infinite else 0.0)
+    uniform = torch.rand(rows, generator=gen, device="cuda")
+    tokens, logprobs = torch.empty(rows, dtype=torch.int64, device="cuda"), torch.empty(rows, device="cuda")
+    for _ in range(30):
+        tokens.fill_(-7)
+        ops.sample(logits, None, None, None, None, uniform, tokens, logprobs)
+        assert torch.equal(tokens, best[:, 0]) and int(torch.count_nonzero(logprobs)) == 0
