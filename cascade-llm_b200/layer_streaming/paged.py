@@ -176,8 +176,12 @@ class PagedBatchDecoder:
         return state.logits.view(-1)
 
     def fork(self, parents, children):
+        parents, children = _slots(parents, self.device), _slots(children, self.device)
         self.cache.fork(parents, children)
-        self.tokens[_slots(children, self.device).long()] = self.tokens[_slots(parents, self.device).long()]
+        # a refused fork (cache.status, on the device) may name slots that do not exist: it indexes
+        # existing ones and leaves their tokens
+        source, target = (slots.clamp(0, self.sequences - 1).long() for slots in (parents, children))
+        self.tokens[target] = torch.where(self.cache.status == 0, self.tokens[source], self.tokens[target])
 
     def free(self, slots):
         self.cache.free(slots)
