@@ -3,11 +3,13 @@
 //
 // Token n at position p, rotary frequency f_i, pair (a, b) of a head:
 //   (a, b) -> c * (a cos(p f_i) - b sin(p f_i), b cos(p f_i) + a sin(p f_i)).
-// The angle p * f_i is formed in double (exact for every int32 position) and
-// split into a 32-bit part and its remainder, which corrects sine and cosine
-// to second order: a 32-bit product alone is off by up to half an ulp of the
-// angle, 0.004 rad at position 100,000. The rotation runs in 32 bits and is
-// rounded once, to the cache's type.
+// The angle p * f_i has up to 55 bits and its whole turns tell nothing: it is formed
+// as a double and the product's rounding error, and reduced to [-pi, pi] with 2 pi
+// in two parts (Cody and Waite's reduction), then split into a 32-bit part and its
+// remainder, which corrects sine and cosine to first order. A 32-bit angle is off by
+// up to half an ulp, 0.004 rad at position 100,000 and 64 rad at 2^31; this is right
+// to 2^-22 at every int32 position (frequencies up to 2^20). The rotation runs in
+// 32 bits and is rounded once, to the cache's type.
 //
 // The work is moving 16-bit values once in and once out (HBM-bound; for a
 // decode step of a few tokens it is launch latency). One CTA per token: its
@@ -38,6 +40,8 @@ struct AppendParams {
 // tokens 35 us = 5.8 TB/s, 41 with 384).
 constexpr int kAppendFew = 384, kAppendMany = 128;
 constexpr int kMaxRotary = 512;
+// 2 pi as a double and what it leaves out (2 pi = 6.283185307179586476925286766559005768...)
+constexpr double kTurnHigh = 6.283185307179586, kTurnLow = 2.4492935982947064e-16, kTurnsPerRadian = 1.0 / kTurnHigh;
 
 template <typename T>
 __global__ void __launch_bounds__(kAppendFew) paged_append_kernel(const __grid_constant__ AppendParams p) {
@@ -61,12 +65,13 @@ __global__ void __launch_bounds__(kAppendFew) paged_append_kernel(const __grid_c
   }
   const int half = p.rotary >> 1;
   for (int i = threadIdx.x; i < half; i += blockDim.x) {
-    const double angle = double(p.inv_freq[i]) * double(pos);
+    const double f = double(p.inv_freq[i]), product = f * double(pos), rest = fma(f, double(pos), -product);
+    const double turns = rint(product * kTurnsPerRadian);
+    const double angle = fma(-turns, kTurnHigh, product) + fma(-turns, kTurnLow, rest);
     const float hi = float(angle), lo = float(angle - double(hi));
     float s, c;
     sincosf(hi, &s, &c);
-    const float even = fmaf(-0.5f * lo, lo, 1.0f);  // cos(lo); sin(lo) = lo to this order
-    turn[i] = make_float2((c * even - s * lo) * p.factor, (s * even + c * lo) * p.factor);
+    turn[i] = make_float2((c - s * lo) * p.factor, (s + c * lo) * p.factor);
   }
   __syncthreads();
 

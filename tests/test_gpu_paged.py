@@ -430,3 +430,21 @@ def test_append_then_attention_in_a_graph_on_a_side_stream(workspace):
         side.synchronize()
     want, _, weight, _ = oracle.attention(q_out.cpu(), k_pages.cpu(), v_pages.cpu(), table.cpu(), lengths.cpu(), scale)
     assert ((out.cpu().double() - want).abs() <= 2.05 * 2.0 ** -8 * weight + 1e-6).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_at_any_int32_position(cuda, dtype, interleaved):
+    """The largest angle is the position itself, which 32 bits hold to within 64 rad at 2^31."""
+
+    position = [0, 1048577, 4194303, 7000001, 16777217, 123456789, 2 ** 30 + 1, 2 ** 31 - 2 ** 16 - 1]
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    qkv = torch.randn((len(position), 4, 64), generator=gen, device="cuda").to(dtype)
+    page = 1 << 16
+    table = torch.full((1, 2 ** 31 // page - 1), -1, dtype=torch.int32)
+    for n, j in enumerate(position):
+        table[0, j // page] = n
+    pool = lambda: torch.zeros((len(position), 1, page, 64), dtype=dtype, device="cuda")  # noqa: E731
+    sequence = torch.zeros(len(position), dtype=torch.int32, device="cuda")
+    _check_append(qkv[:, :2], qkv[:, 2:3], qkv[:, 3:], sequence, torch.tensor(position, dtype=torch.int32, device="cuda"),
+                  table.cuda(), pool(), pool(), 64, interleaved)
