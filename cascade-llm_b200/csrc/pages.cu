@@ -56,6 +56,17 @@ __device__ __forceinline__ int block_scan(int v, int* part, int& total) {
   return before + x - v;
 }
 
+// Sum of one value per thread over the CTA, for every thread.
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* part) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0;
+  for (int w = 0; w < int(blockDim.x >> 5); ++w) v += part[w];
+  return v;
+}
+
 // The pages [first, last) that this warp owns.
 __device__ __forceinline__ void warp_pages(int pages, int& first, int& last) {
   const int per = ((pages + int(blockDim.x) - 1) / int(blockDim.x)) * 32, warp = threadIdx.x >> 5;
@@ -276,6 +287,7 @@ struct ReserveParams {
 
 __global__ void __launch_bounds__(kPlanThreads) pages_reserve_kernel(const __grid_constant__ ReserveParams p) {
   __shared__ int part[kPlanWarps];
+  __shared__ int64_t sums[kPlanWarps];
   __shared__ int first[kPlanThreads], held[kPlanThreads], want[kPlanThreads];
   __shared__ Picks picks;
   __shared__ int bad;
@@ -286,27 +298,22 @@ __global__ void __launch_bounds__(kPlanThreads) pages_reserve_kernel(const __gri
   __syncthreads();
   int64_t need = 0;
   bool wrong = false;
-  for (int base = 0; base < p.sequences; base += threads) {
-    const int s = base + tid;
-    int more = 0, total;
-    if (s < p.sequences) {
-      const int64_t length = p.lengths[s], grown = length + p.extra[s];
-      if (length < 0 || p.extra[s] < 0 || grown > int64_t(p.width) * p.page_size)
-        wrong = true;
-      else
-        more = page_count(grown, p.page_size) - page_count(length, p.page_size);
-    }
-    // more than all pages is refused below; the clamp keeps the sum in range
-    block_scan(min(more, p.pages + 1), part, total);
-    need += total;
-    if (need > p.pages) need = int64_t(p.pages) + 1;
+  for (int s = tid; s < p.sequences; s += threads) {
+    const int64_t length = p.lengths[s], grown = length + p.extra[s];
+    if (length < 0 || p.extra[s] < 0 || grown > int64_t(p.width) * p.page_size)
+      wrong = true;
+    else
+      need += page_count(grown, p.page_size) - page_count(length, p.page_size);
   }
+  need = block_sum(need, sums);
   if (wrong) bad = 1;
   __syncthreads();
   const bool stop = bad != 0;
-  const int free = pick_free(p.ref, p.pages, stop ? 0 : int(need), open, picks, p.workspace, part);
-  if (stop || free < need) {
-    if (tid == 0) p.status[0] = stop ? -1 : int(need) - free;
+  // (more than all pages can never be picked: the exact need is only told)
+  const int wanted = int(min(need, int64_t(p.pages) + 1));
+  const int free = pick_free(p.ref, p.pages, stop ? 0 : wanted, open, picks, p.workspace, part);
+  if (stop || free < wanted) {
+    if (tid == 0) p.status[0] = stop ? -1 : int(min(need - free, int64_t(INT32_MAX)));
     return;
   }
   int before = 0;
@@ -454,7 +461,7 @@ static int plan_threads(int pages, int requests) {
 }
 static int check_state(const char* what, const void* table, int sequences, int width, const void* ref, int pages) {
   CB_REQUIRE(sequences >= 1 && width >= 1 && pages >= 1, "%s: sequences, table width and pages must be positive", what);
-  // the plan kernels' 32-bit scans add up to 1024 counts of at most pages + 1
+  // the plan kernels' 32-bit scans add up to 1024 counts of at most pages
   CB_REQUIRE(pages <= kMaxPages, "%s: pages=%d (at most %d)", what, pages, kMaxPages);
   CB_REQUIRE(table && ref, "%s: null pointer", what);
   return kOk;

@@ -404,8 +404,8 @@ int cb_paged_attention(const void* q, int64_t q_token, int64_t q_head, const voi
 
 /* Page bookkeeping. Free pages are taken lowest index first, in the order of
  * the request, so a result is determined by the state. fork and reserve are
- * all or nothing: status[0] = 0 done; > 0: that many pages are missing; -1:
- * an argument is wrong (index out of range, a child that is not empty, listed
+ * all or nothing: status[0] = 0 done; > 0: that many pages are missing
+ * (at most 2^31 - 1 is told); -1: an argument is wrong (index out of range, a child that is not empty, listed
  * twice or also a parent, a row too narrow, a negative length or extra); a
  * status other than 0 leaves the state as it was. workspace:
  * cb_pages_workspace_ints(pages) int32 of scratch. pages <= 2000000; fork:

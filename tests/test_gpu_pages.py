@@ -241,3 +241,18 @@ def test_refusals(cuda):
         with pytest.raises((ValueError, TypeError, RuntimeError)):
             call()
     d.check(o)
+
+
+def test_reserve_counts_what_is_missing_beyond_the_whole_pool(cuda):
+    o = _state([10, 0, 30], 13, 3000, 4)
+    d = Device(o)
+    assert _reserve(d, o, [0, 80, 0]) == 18  # 20 pages, 2 free
+    assert _reserve(d, o, [4000, 0, 9000]) == 3248
+    assert _reserve(d, o, [2, 8, 2]) == 0
+
+
+def test_reserve_counts_what_many_sequences_miss(cuda):
+    o = _state([0] * 1500, 20, 300, 1)
+    d = Device(o)
+    assert _reserve(d, o, [s % 300 for s in range(1500)]) == 5 * 299 * 150 - 20
+    assert _reserve(d, o, [300] * 1500) == 450000 - 20
