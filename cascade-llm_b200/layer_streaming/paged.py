@@ -148,10 +148,14 @@ class PagedBatchDecoder:
     # ---------------------------------------------------------------- prompts
     def add(self, prompt_ids, slot):
         """Run a prompt (int64 [1, n]) and keep it in an empty slot; returns the
-        logits behind its last token, fp32 [vocab]."""
+        logits behind its last token, fp32 [vocab]. If it fails, the slot stays
+        empty; an earlier refused fork or step that nobody has read is raised
+        before anything is taken."""
 
         if not 0 <= int(slot) < self.sequences:
             raise ValueError("slot {} is not one of {}".format(slot, self.sequences))
+        if prompt_ids.dim() != 2 or prompt_ids.shape[0] != 1 or prompt_ids.shape[1] < 1:
+            raise ValueError("a prompt must be [1, tokens] (got {})".format(list(prompt_ids.shape)))
         ex, cache = self.executor, self.cache
         if int(cache.lengths[slot]):
             raise ValueError("slot {} is in use".format(slot))
@@ -159,20 +163,27 @@ class PagedBatchDecoder:
         if length > cache.max_length:
             raise ValueError("a prompt of {} tokens passes max_length={}".format(length, cache.max_length))
         with torch.cuda.device(self.device), torch.inference_mode():
+            cache.check()
             extra = torch.zeros(self.sequences, dtype=torch.int32, device=self.device)
             extra[slot] = length
             cache.reserve(extra)
             cache.check()
-            ex.kv_cache.clear()
-            state = ex.finish(self.runtime.run(ex, ex.begin(prompt_ids)))
-            position = torch.arange(length, dtype=torch.int32, device=self.device)
-            sequence = torch.full((length,), int(slot), dtype=torch.int32, device=self.device)
-            for layer in range(ex.config.num_hidden_layers):
-                # the executor's keys are rotated already: [heads, n, dim] read as tokens
-                key, value = (part[:, :length].transpose(0, 1) for part in (ex.kv_cache.key(layer),
-                                                                             ex.kv_cache.value(layer)))
-                ops.paged_append(None, key, value, None, position, sequence, cache.table, None, *cache.layer(layer))
-            ex.kv_cache.clear()
+            try:
+                ex.kv_cache.clear()
+                state = ex.finish(self.runtime.run(ex, ex.begin(prompt_ids)))
+                position = torch.arange(length, dtype=torch.int32, device=self.device)
+                sequence = torch.full((length,), int(slot), dtype=torch.int32, device=self.device)
+                for layer in range(ex.config.num_hidden_layers):
+                    # the executor's keys are rotated already: [heads, n, dim] read as tokens
+                    key, value = (part[:, :length].transpose(0, 1) for part in (ex.kv_cache.key(layer),
+                                                                                 ex.kv_cache.value(layer)))
+                    ops.paged_append(None, key, value, None, position, sequence, cache.table, None,
+                                     *cache.layer(layer))
+            except BaseException:
+                cache.free([slot])
+                raise
+            finally:
+                ex.kv_cache.clear()
         return state.logits.view(-1)
 
     def fork(self, parents, children):
