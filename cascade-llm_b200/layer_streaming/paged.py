@@ -289,19 +289,23 @@ class PagedBatchDecoder:
     def best_of(self, prompt_ids, new_tokens, generator=None, temperature=1.0, top_k=None, top_p=None, min_p=None):
         """`sequences` sampled continuations of one prompt: (tokens int64
         [sequences, new_tokens], log probabilities fp32 of the same shape). The
-        prompt's full pages are shared; slots must be empty and are empty again
-        at the end."""
+        prompt's full pages are shared; every slot must be empty and is empty
+        again at the end, also of a call that fails."""
 
         if new_tokens < 1:
             raise ValueError("new_tokens must be positive")
+        used = self.cache.lengths.nonzero().flatten().tolist()
+        if used:
+            raise ValueError("best_of needs every slot: {} are in use".format(used))
         others = list(range(1, self.sequences))
         tokens, logprobs = [], []
         filters = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         uniform = torch.empty(self.sequences, device=self.device)
-        logits = self.add(prompt_ids, 0).view(1, -1).expand(self.sequences, -1)
-        if others:
-            self.fork([0] * len(others), others)
         try:
+            logits = self.add(prompt_ids, 0).view(1, -1).expand(self.sequences, -1)
+            if others:
+                self.fork([0] * len(others), others)
+                self.cache.check()
             for i in range(new_tokens):
                 uniform.uniform_(generator=generator)
                 picked, probability = self.sample(logits, uniform, **filters)
