@@ -56,7 +56,8 @@ class PagedKVCache:
         self.page_size = int(page_size)
         width = -(-int(max_length) // self.page_size)
         ints = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=self.device)  # noqa: E731
-        self.storage = torch.empty((layer_count, 2, pages, kv_heads, page_size, head_dim), dtype=dtype,
+        # zeros: what nobody has written is then the same in every cache (torch.empty gives a NaN at times)
+        self.storage = torch.zeros((layer_count, 2, pages, kv_heads, page_size, head_dim), dtype=dtype,
                                    device=self.device)
         self.table = torch.full((sequences, width), -1, dtype=torch.int32, device=self.device)
         self.lengths, self.ref, self.status = ints(sequences), ints(pages), ints(1)
