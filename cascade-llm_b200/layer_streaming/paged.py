@@ -140,6 +140,8 @@ class PagedBatchDecoder:
             self.logits = new(executor.config.vocab_size)
             self.tokens = torch.zeros(rows, dtype=torch.int64, device=self.device)
             self.logprobs = torch.zeros(rows, dtype=torch.float32, device=self.device)
+            self._picked = torch.empty(rows, dtype=torch.int64, device=self.device)
+            self._no_choice = torch.zeros(rows, dtype=torch.bool, device=self.device)  # since the last check
             self._position = torch.empty(rows, dtype=torch.int32, device=self.device)
             self._extra = torch.empty(rows, dtype=torch.int32, device=self.device)
             self._attention_ws = torch.zeros(ops.paged_attention_workspace_bytes(), dtype=torch.uint8,
@@ -266,7 +268,9 @@ class PagedBatchDecoder:
     def sample(self, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
         """The next token of every slot into ``tokens`` (and its log probability
         into ``logprobs``) from uniform numbers in [0, 1); parameters: one value
-        for all slots, or one per slot."""
+        for all slots, or one per slot. A slot whose logits leave no choice
+        (all NaN or -inf) keeps its token, at a log probability of -inf;
+        :meth:`check_errors` raises if it holds a sequence."""
 
         def per_slot(value, dtype):
             if value is None:
@@ -276,16 +280,23 @@ class PagedBatchDecoder:
 
         with torch.cuda.device(self.device), torch.inference_mode():
             ops.sample(logits, per_slot(temperature, torch.float32), per_slot(top_k, torch.int32),
-                       per_slot(top_p, torch.float32), per_slot(min_p, torch.float32), uniform, self.tokens,
+                       per_slot(top_p, torch.float32), per_slot(min_p, torch.float32), uniform, self._picked,
                        self.logprobs)
-            self.tokens.clamp_(min=0)  # -1: a row without a choice (an empty slot's logits may be anything)
+            none = self._picked < 0
+            self._no_choice.logical_or_(none & (self.cache.lengths > 0))
+            self.tokens.copy_(torch.where(none, self.tokens, self._picked))
         return self.tokens, self.logprobs
 
     def check_errors(self):
-        """Raise if a step ran out of pages or a kernel reported a bad index."""
+        """Raise if a step ran out of pages, a sequence had no token to choose
+        from, or a kernel reported a bad index."""
 
+        no_choice = self._no_choice.nonzero().flatten().tolist()
+        self._no_choice.zero_()
         self.cache.check()
         self.executor.check_errors()
+        if no_choice:
+            raise RuntimeError("slots {} had no token to choose from: all logits NaN or -inf".format(no_choice))
 
     def best_of(self, prompt_ids, new_tokens, generator=None, temperature=1.0, top_k=None, top_p=None, min_p=None):
         """`sequences` sampled continuations of one prompt: (tokens int64
