@@ -119,7 +119,7 @@ class PagedBatchDecoder:
     ``executor`` (a Llama31DecodeExecutor with the vocabulary resident) and
     ``runtime`` (``weights="hbm"``) supply the weights and run the prompts; the
     executor's own request is given up while a prompt is added. Slots that are
-    empty take part as padding: their logits mean nothing.
+    empty take part as padding.
     """
 
     def __init__(self, executor, runtime, sequences, pages, max_length, page_size=16, use_graphs=True):
@@ -142,6 +142,7 @@ class PagedBatchDecoder:
             self.logprobs = torch.zeros(rows, dtype=torch.float32, device=self.device)
             self._picked = torch.empty(rows, dtype=torch.int64, device=self.device)
             self._no_choice = torch.zeros(rows, dtype=torch.bool, device=self.device)  # since the last check
+            self._full = torch.zeros(rows, dtype=torch.bool, device=self.device)  # the same
             self._position = torch.empty(rows, dtype=torch.int32, device=self.device)
             self._extra = torch.empty(rows, dtype=torch.int32, device=self.device)
             self._attention_ws = torch.zeros(ops.paged_attention_workspace_bytes(), dtype=torch.uint8,
@@ -239,18 +240,28 @@ class PagedBatchDecoder:
 
     def _step(self):
         ex, cache = self.executor, self.cache
-        torch.gt(cache.lengths, 0, out=self._extra)
+        full = cache.lengths >= cache.max_length  # stops alone: a reserve is all or nothing
+        self._full.logical_or_(full)
+        self._extra.copy_((cache.lengths > 0) & ~full)
         cache.reserve(self._extra)
         # a refused reserve leaves the lengths as they were: nothing may be written then
-        self._position.copy_(torch.where(cache.status == 0, cache.lengths - 1, -1))
+        went = (cache.status == 0) & (self._extra > 0)
+        self._position.copy_(torch.where(went, cache.lengths - 1, -1))
         ops.embedding(self.tokens, ex.resident["model.embed_tokens.weight"], self._x)
         self._layers()
         ops.rmsnorm(self._x, ex.resident["model.norm.weight"], ex.eps, self._xn)
         ops.gemm_bf16(self._xn, ex.resident["lm_head.weight"], self.logits)
+        self.logits.masked_fill_(~went.unsqueeze(1), float("nan"))
 
     def step(self):
         """Append every slot's token (``tokens``) to its sequence; the logits
-        behind them, bf16 [sequences, vocab]."""
+        behind them, bf16 [sequences, vocab] (the next step's go to the same
+        memory).
+
+        Slots that took no step have NaN logits, from which :meth:`sample`
+        leaves their tokens as they are: empty ones, those at ``max_length``,
+        and all of them where pages ran out. Such a step can be taken again
+        once pages are free; :meth:`check_errors` tells of it."""
 
         with torch.cuda.device(self.device), torch.inference_mode():
             if not self.use_graphs:
@@ -288,13 +299,18 @@ class PagedBatchDecoder:
         return self.tokens, self.logprobs
 
     def check_errors(self):
-        """Raise if a step ran out of pages, a sequence had no token to choose
-        from, or a kernel reported a bad index."""
+        """Raise if a step ran out of pages or found a sequence at
+        ``max_length``, a sequence had no token to choose from, or a kernel
+        reported a bad index."""
 
-        no_choice = self._no_choice.nonzero().flatten().tolist()
+        full, no_choice = (flags.nonzero().flatten().tolist() for flags in (self._full, self._no_choice))
+        self._full.zero_()
         self._no_choice.zero_()
         self.cache.check()
         self.executor.check_errors()
+        if full:
+            raise ValueError("slots {} took no step: they hold max_length={} tokens".format(
+                full, self.cache.max_length))
         if no_choice:
             raise RuntimeError("slots {} had no token to choose from: all logits NaN or -inf".format(no_choice))
 
