@@ -10,6 +10,7 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import sys
 import threading
 
 import torch
@@ -202,7 +203,7 @@ def load_binding():
     if not os.path.exists(path):
         raise RuntimeError(
             "cascade_binding.so not found at {} - build it with "
-            "`make -C cascade-llm_b200/csrc` (or __graft_entry__.build())".format(path)
+            "`make -C cascade-llm_b200/csrc PYTHON={}` (or __graft_entry__.build())".format(path, sys.executable)
         )
     loader = importlib.machinery.ExtensionFileLoader("cascade_binding", path)
     module = importlib.util.module_from_spec(importlib.util.spec_from_loader("cascade_binding", loader))

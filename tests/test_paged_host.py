@@ -1,7 +1,10 @@
 """Paged serving without a GPU: the binding loads and refuses, the entry points
 refuse before any launch, and the oracle keeps the page bookkeeping's invariants."""
 
+import os
 import random
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -133,3 +136,18 @@ def test_oracle_attention_and_rotation_on_a_small_case():
         torch.testing.assert_close(y.square().sum(-1), x.double().square().sum(-1))  # a rotation
         back = oracle.rotate(y, freq, -position, interleaved)
         torch.testing.assert_close(back, x.double())
+
+
+def test_the_library_builds_without_torch():
+    """A user of the C interface alone needs neither Python's nor torch's headers."""
+
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cascade-llm_b200", "csrc")
+
+    def planned(python):
+        run = subprocess.run(["make", "-n", "-B", "-C", csrc, "PYTHON=" + python], capture_output=True, text=True)
+        assert run.returncode == 0, run.stderr
+        return run.stdout
+
+    for python in ("/nowhere/python3", sys.executable + " -S -I"):  # no Python; one without its packages
+        assert "libcascade_b200.so" in planned(python) and "cascade_binding.so" not in planned(python)
+    assert "libcascade_b200.so" in planned(sys.executable) and "cascade_binding.so" in planned(sys.executable)
