@@ -22,6 +22,8 @@ copied into pages. Every step has fixed shapes and keeps lengths, tables and
 free pages on the device, so it is captured once and replayed as a CUDA graph.
 """
 
+import warnings
+
 import torch
 
 from . import _native, ops
@@ -127,6 +129,9 @@ class PagedBatchDecoder:
             raise ValueError("the paged decoder needs HBM-resident weights (weights='hbm')")
         if executor.vocab_runtime is not None:
             raise ValueError("the paged decoder needs the vocabulary resident")
+        if executor.decode_weights != "bf16":
+            warnings.warn("decode_weights={!r} is for the executor's own one-token steps: the paged steps read the "
+                          "bf16 weights".format(executor.decode_weights), stacklevel=2)
         self.executor, self.runtime, self.device = executor, runtime, executor.device
         self.sequences = int(sequences)
         self.cache = PagedKVCache(sequences, pages, max_length, executor.config.num_hidden_layers,
