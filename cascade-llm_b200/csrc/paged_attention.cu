@@ -28,8 +28,9 @@
 //   mma.sync rather than tcgen05: the latter's smallest tile has 64 rows, and at
 //   these ratios the tensor pipe is idle most of the time either way.
 // * Softmax statistics and sums are fp32. P enters the second product as the
-//   sum of two 16-bit values (rounded, and the rest), which keeps its rounding
-//   out of the result.
+//   sum of two 16-bit values (rounded, and the rest): weights to 2^-16 (bf16) or
+//   2^-22 (fp16), where one value leaves 2^-8 or 2^-11. The output's own rounding
+//   hides that but for 1 to 3 in 1000 outputs, which differ in their last place.
 //
 // Measured: 858,000 positions of 8 KV heads x 128 in 530 us = 6.7 TB/s (a plain copy
 // moves 6.5); 32 sequences of 1 to 4096 positions 17 us; one of 77 4.6 us.

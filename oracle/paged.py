@@ -47,6 +47,61 @@ def attention(q, k_pages, v_pages, table, lengths, scale):
     return out, lse, weight, size
 
 
+def cancelling_case(dtype, head_dim, group, lengths, page):
+    """(q, k_pages, v_pages, table, lengths) of one KV head whose outputs nearly vanish although
+    their terms do not: an error of the softmax weights stands out of the outputs' own rounding.
+
+    Scores (at a scale of 1) are 0 at even positions and -a_h at odd ones, exact in any
+    arithmetic; the weights there are 1 and e^-a_h. Values are 1 at odd positions and, at even
+    ones, -e^-a_h rounded to the type, for head h = dimension modulo the group."""
+
+    a = (0.15 + 2.7 * torch.arange(group, dtype=torch.float64) / group).to(dtype)
+    counts = [-(-n // page) for n in lengths]
+    pages, width = sum(counts) + 1, max(counts)
+    q = torch.zeros((len(lengths), group, head_dim), dtype=dtype)
+    q[:, :, 0] = a
+    k = torch.randn((pages, 1, page, head_dim), generator=torch.Generator().manual_seed(2)).to(dtype)
+    v = torch.empty_like(k)
+    table = torch.full((len(lengths), width), -1, dtype=torch.int32)
+    near = torch.exp(-a.double()).to(dtype)[torch.arange(head_dim) % group]
+    first = 0
+    for b, n in enumerate(lengths):
+        for j in range(counts[b] * page):
+            at = pages - 1 - first - j // page
+            table[b, j // page] = at
+            k[at, 0, j % page, 0] = -(j % 2)
+            v[at, 0, j % page] = 1.0 if j % 2 else -near
+        first += counts[b]
+    return q, k, v, table, torch.tensor(lengths, dtype=torch.int32)
+
+
+def cancelling_bound(dtype, want, weight, lengths):
+    """What such an output may be off by: its own rounding (u |o|, 2^-25 among fp16's subnormals), weights
+    in two parts of the type (u^2), the 32-bit exponent's argument (6 at most, 10 more where fp16's weights
+    are lifted: 2^-19 in all) and the 32-bit sums of two products per position and of the weights."""
+
+    u = UNIT[dtype]
+    sums = (3 * lengths.double() + 16)[:, None, None] * 2.0 ** -23
+    return 1.01 * u * want.abs() + (1.01 * u * u + 2.0 ** -19 + sums) * weight + 2.0 ** -25
+
+
+def attention_in_parts(q, k_pages, v_pages, table, lengths, parts):
+    """The outputs at a scale of 1 with weights held as `parts` values of q's type, else in 64 bits."""
+
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    page = k_pages.shape[2]
+    for b, length in enumerate(lengths.tolist()):
+        held = table[b, :-(-length // page)].long()
+        k, v = (x[held, 0].double().reshape(-1, q.shape[2])[:length] for x in (k_pages, v_pages))
+        p = torch.exp(q[b].double() @ k.t())
+        p = p / p.amax(-1, keepdim=True)
+        kept = torch.zeros_like(p)
+        for _ in range(parts):
+            kept += (p - kept).to(q.dtype).double()
+        out[b] = kept @ v / p.sum(-1, keepdim=True)
+    return out
+
+
 class Pages:
     """The bookkeeping on Python lists, page contents included: content[p] is
     any value that stands for page p."""

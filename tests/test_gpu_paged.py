@@ -448,3 +448,14 @@ def test_append_at_any_int32_position(cuda, dtype, interleaved):
     sequence = torch.zeros(len(position), dtype=torch.int32, device="cuda")
     _check_append(qkv[:, :2], qkv[:, 2:3], qkv[:, 3:], sequence, torch.tensor(position, dtype=torch.int32, device="cuda"),
                   table.cuda(), pool(), pool(), 64, interleaved)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("d,group", [(64, 3), (128, 8), (128, 16), (64, 16)])
+def test_attention_weights_are_not_rounded_to_the_cache_type(workspace, dtype, d, group):
+    """Outputs that nearly vanish: the bound leaves no room for weights of 8 or 11 bits."""
+
+    case = oracle.cancelling_case(dtype, d, group, [16, 32, 48, 2], 24)
+    want, _, weight, _ = oracle.attention(*case, 1.0)
+    out, _ = _run_attention(*(x.cuda() for x in case), workspace, scale=1.0)
+    assert ((out.cpu().double() - want).abs() <= oracle.cancelling_bound(dtype, want, weight, case[-1])).all()

@@ -151,3 +151,14 @@ def test_the_library_builds_without_torch():
     for python in ("/nowhere/python3", sys.executable + " -S -I"):  # no Python; one without its packages
         assert "libcascade_b200.so" in planned(python) and "cascade_binding.so" not in planned(python)
     assert "libcascade_b200.so" in planned(sys.executable) and "cascade_binding.so" in planned(sys.executable)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("head_dim,group", [(64, 3), (128, 8), (128, 16)])
+def test_the_cancelling_case_tells_weights_in_one_part_from_two(dtype, head_dim, group):
+    q, k, v, table, lengths = oracle.cancelling_case(dtype, head_dim, group, [16, 32, 48, 2], 24)
+    want, _, weight, _ = oracle.attention(q, k, v, table, lengths, 1.0)
+    bound = oracle.cancelling_bound(dtype, want, weight, lengths)
+    one, two = (oracle.attention_in_parts(q, k, v, table, lengths, parts) for parts in (1, 2))
+    assert bool(((one - want).abs() > 2 * bound).any(-1).any(-1).all())  # planted: the rest of each weight dropped
+    assert bool(((two - want).abs() <= 0.5 * bound).all())
