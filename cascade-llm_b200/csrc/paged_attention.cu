@@ -69,11 +69,13 @@ constexpr int kMaxRows = 16;                // query heads of a CTA's segment
 // without it, 18 with 1 or 2, 18.7 with 3.
 constexpr int kSegmentCost = 2;
 // A CTA's share at least, in places: parts cost 2 us for the ticket and 0.1 to
-// 0.2 us each for the join. One sequence of 77 positions 6.7 / 5.2 / 9.5 us with 1 /
-// 4 / 6, of 2048 10.5 / 11.1 / 12.9; 64-wide heads (half the bytes per unit), 18
-// sequences of 33 to 9001 positions, 21.0 / 17.7 / 15.5.
-template <int D>
-constexpr int kShareMin = D == 64 ? 6 : 4;
+// 0.2 us each for the join, the units of a share follow one another. With 1 / 2 / 4 /
+// 8: one sequence of 77 positions (32 query and 8 KV heads of 128) 6.4 / 4.6 / 4.6 /
+// 7.3 us, of 2048 12.0 / 10.4 / 10.9 / 14.1, of 32,000 32 with each; of 8 and 2 heads of
+// 64 5.9 / 4.1 / 4.1 / 6.4, 7.8 / 7.3 / 8.7 / 11.5 and 24.3 / 24.4 / 22.2 / 17.7; 12 of
+// 100 to 20,000, 8 heads over one of 64, 20.1 / 20.2 / 17.4 / 15.9. Short sequences
+// want less, long ones of few KV heads more.
+constexpr int kShareMin = 4;
 constexpr int kTicketBytes = 4096;
 
 template <int D>
@@ -222,7 +224,7 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtas) paged_attention_ker
   total *= heads;
   before *= heads;
   own *= heads;
-  const int ctas = int(min(Place(gridDim.x), (total + kShareMin<D> - 1) / kShareMin<D>));
+  const int ctas = int(min(Place(gridDim.x), (total + kShareMin - 1) / kShareMin));
   if (int(blockIdx.x) >= ctas) return;
   const Shares<Place> shares(total, ctas);
   const Place v0 = shares.begin(blockIdx.x), v1 = shares.begin(blockIdx.x + 1);
