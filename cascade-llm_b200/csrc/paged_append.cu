@@ -37,7 +37,7 @@ struct AppendParams {
 
 // Threads of a token's CTA: one wave of CTAs takes more (an item each at 48 heads
 // of 128; 64 tokens 2.8 us, 3.8 with 128 threads), a long prompt fewer (8193
-// tokens 35 us = 5.8 TB/s, 41 with 384).
+// tokens 35 us = 5.7 TB/s in a graph, 41 with 384).
 constexpr int kAppendFew = 384, kAppendMany = 128;
 constexpr int kMaxRotary = 512;
 // 2 pi as a double and what it leaves out (2 pi = 6.283185307179586476925286766559005768...)

@@ -32,8 +32,9 @@
 //   2^-22 (fp16), where one value leaves 2^-8 or 2^-11. The output's own rounding
 //   hides that but for 1 to 3 in 1000 outputs, which differ in their last place.
 //
-// Measured: 858,000 positions of 8 KV heads x 128 in 530 us = 6.7 TB/s (a plain copy
-// moves 6.5); 32 sequences of 1 to 4096 positions 17 us; one of 77 4.6 us.
+// Measured: 858,000 positions of 8 KV heads x 128 in 523 us = 6.8 TB/s (a plain copy
+// moves 6.5); 32 sequences of 1 to 4096 positions 19.8 us (17.5 with the pages in L2);
+// one of 77 4.5 us.
 #include "cascade_b200.h"
 #include "internal.h"
 #include "paged_device.cuh"
@@ -64,9 +65,10 @@ constexpr int kUnit = kTile * kPagedWarps;  // positions of a CTA's step
 constexpr int kStages = 3;
 constexpr int kPagedCtas = 2;               // per SM
 constexpr int kMaxRows = 16;                // query heads of a CTA's segment
-// Beginning and ending a segment (its queries, the join of the warps) takes
-// about as long as this many units: 32 sequences of 1 to 4096 positions 24.4 us
-// without it, 18 with 1 or 2, 18.7 with 3.
+// Beginning and ending a segment (its queries, the join of the warps) takes about as
+// long as this many units. With 0 / 1 / 2 / 3: 32 sequences of 1 to 4096 positions
+// 21.4 / 19.9 / 19.7 / 20.2 us, 100 of 10 to 800 26.0 / 22.7 / 23.8 / 25.4, one of 77
+// 7.3 / 8.9 / 4.5 / 6.4.
 constexpr int kSegmentCost = 2;
 // A CTA's share at least, in places: parts cost 2 us for the ticket and 0.1 to
 // 0.2 us each for the join, the units of a share follow one another. With 1 / 2 / 4 /

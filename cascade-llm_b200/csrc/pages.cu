@@ -13,9 +13,9 @@
 // kernel moves the pages' bytes (HBM-bound: read + write of outer x page_bytes
 // per page) and edits table rows; it reads the plan's outcome on the device.
 //
-// Measured: half of 1024 pages of 2 MB compacted in 177 us = 6.0 TB/s read and
+// Measured: half of 1024 pages of 2 MB compacted in 183 us = 5.8 TB/s read and
 // written (a plain copy: 6.5); a fork of 7 children with their tails 9 us, a free
-// 1.1, a reserve 3.1: one chain of loads and a few barriers each.
+// 1.1, a reserve 3.0: one chain of loads and a few barriers each.
 #include "cascade_b200.h"
 #include "internal.h"
 #include "paged_device.cuh"

@@ -35,9 +35,12 @@
 // (a logit, and how many that equal it), and the cluster searches its slices in index
 // order, as it does where nothing filters.
 //
-// Measured: one row of 128256 fp32 logits 4.7 us greedy, 12.8 with top-k 50, 18 with
-// top-p 0.9 (39 over flat logits); 256 bf16 rows 10.7 greedy, 28 with top-k 50, 60 with
-// mixed filters (their floor, one read, is 10).
+// Measured with logits from HBM (in L2): one row of 128256 fp32 logits 6.0 us (4.6)
+// greedy, 14 (13) with top-k 50, 17 to 40 with top-p 0.9, by the number of tokens that it
+// keeps; 256 bf16 rows 15 (11) greedy, 33 (28) with top-k 50, 53 (47) unfiltered, 66 (59)
+// with mixed filters, where one read from HBM takes 10. Times beside the choices below
+// are with the logits in L2. Registers: 64, the most for two CTAs per SM, with 256 to 316
+// bytes of spill stores: one kernel holds every path.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 

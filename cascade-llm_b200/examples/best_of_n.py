@@ -1,4 +1,5 @@
-"""Best of n: n sampled continuations of one prompt, ranked by mean log probability.
+"""Best of n: n sampled continuations of one prompt, ranked by mean log probability
+(of each token among those that temperature, top-k and top-p kept for it).
 
     python cascade-llm_b200/examples/best_of_n.py [--checkpoint DIR] [--n 8] [--new-tokens 32]
 

@@ -321,7 +321,8 @@ class PagedBatchDecoder:
 
     def best_of(self, prompt_ids, new_tokens, generator=None, temperature=1.0, top_k=None, top_p=None, min_p=None):
         """`sequences` sampled continuations of one prompt: (tokens int64
-        [sequences, new_tokens], log probabilities fp32 of the same shape). The
+        [sequences, new_tokens], log probabilities fp32 of the same shape: among the
+        tokens kept, after temperature and filters, so 0 where one is kept). The
         prompt's full pages are shared; every slot must be empty and is empty
         again at the end, also of a call that fails."""
 
